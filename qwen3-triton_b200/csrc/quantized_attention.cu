@@ -6,6 +6,9 @@
 // scales are, and numerator and denominator keep a running reference each (m, ml). Weights are rounded to fp16 after a
 // factor of 2^15: 11 bits down to 2^-29 of the largest. Integers are exact in fp16; queries in bf16 are taken to fp16 by a
 // power of two per row, and the incomplete block's tokens by one per block. Products accumulate in fp32.
+// The denominator adds up the weights too, block by block, with vs taken out again. A block whose largest weight is below
+// 2^-kFar counts with a larger vs, such that it is 2^-kFar: in fp16 its weights are zero with either, and its share of the
+// denominator does not flush. The last factor 2^{m - ml} / sum reaches beyond fp32's exponents and is applied as two halves.
 #include "quantized_cache.cuh"
 #include "tcgen05.cuh"
 #include <math_constants.h>
@@ -29,6 +32,8 @@ struct AttendParams {
   float scale_log2;
   int* status;
 };
+
+constexpr float kFar = 64.f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -293,6 +298,7 @@ attention_split_kernel(const AttendParams p) {
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         const float nm = fmaxf(m[nt][e], mx);
         ref[e] = nm > -CUDART_INF_F ? nm : 0.f;
+        const float far = mx > -CUDART_INF_F ? fmaxf(ref[e] - kFar - mx, 0.f) : 0.f;     // what log2 vs is raised by
         alpha[e] = exp2_fast(m[nt][e] - ref[e]);
         m[nt][e] = nm;
         float sum = 0.f;
@@ -300,12 +306,12 @@ attention_split_kernel(const AttendParams p) {
         for (int it = 0; it < IT; ++it)
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
-            const float w = exp2_fast(sc[nt][it][2 * hf + e] - (ref[e] - 15.f));
+            const float w = exp2_fast(sc[nt][it][2 * hf + e] - (ref[e] - 15.f - far));
             sc[nt][it][2 * hf + e] = w;
             sum += w;
           }
         if (ahead > 0) {                                           // the same in all lanes of a row
-          const float d = ref[e] - lvs, nml = fmaxf(ml[nt][e], d);
+          const float d = ref[e] - lvs - far, nml = fmaxf(ml[nt][e], d);
           l[nt][e] = l[nt][e] * exp2_fast(ml[nt][e] - nml) + sum * exp2_fast(d - nml);
           ml[nt][e] = nml;
         }
@@ -434,10 +440,10 @@ attention_split_kernel(const AttendParams p) {
   }
   __syncwarp();
 
-  // this warp's sums per row, with their references, into its own ring
+  // this warp's rows, divided by their sums, and log2 of the sums, into its own ring
   constexpr int STRIDE = D + 4;
   float* s_part = reinterpret_cast<float*>(smem + warp * kRingBytes);          // [ROWS][D + 4]
-  float2* s_ref = reinterpret_cast<float2*>(smem + warp * kRingBytes + ROWS * STRIDE * 4);   // log2 of the row's sum, factor of s_part
+  float* s_ref = reinterpret_cast<float*>(smem + warp * kRingBytes + ROWS * STRIDE * 4);     // log2 of the row's sum
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -447,50 +453,55 @@ attention_split_kernel(const AttendParams p) {
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
       const int r = 8 * nt + 2 * t + e;
+      const float whole = ml[nt][e] + log2f(sum), half = sum == 0.f ? 0.f : exp2_fast(0.5f * (m[nt][e] - whole));
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
-        s_part[r * STRIDE + 16 * i + g] = o[nt][i][e];
-        s_part[r * STRIDE + 16 * i + 8 + g] = o[nt][i][2 + e];
+        s_part[r * STRIDE + 16 * i + g] = o[nt][i][e] * half * half;
+        s_part[r * STRIDE + 16 * i + 8 + g] = o[nt][i][2 + e] * half * half;
       }
-      if (g == 0)
-        s_ref[r] = sum == 0.f ? make_float2(-CUDART_INF_F, 0.f) : make_float2(ml[nt][e] + log2f(sum), exp2_fast(m[nt][e] - ml[nt][e]) / sum);
+      if (g == 0) s_ref[r] = sum == 0.f ? -CUDART_INF_F : whole;
     }
   __syncthreads();
   // rows shared out over the warps: the warps' results are weighted by their sums
   constexpr int CPL = D / 32;
   for (int r = warp; r < ROWS && r < p.rows; r += kSplitWarps) {
-    float2 ref[kSplitWarps];
+    // (the weights are divided by their sum before they are used: a sum of large rows may not be finite)
+    float weight[kSplitWarps];
     float mx = -CUDART_INF_F, tot = 0.f, acc[CPL];
 #pragma unroll
     for (int w = 0; w < kSplitWarps; ++w) {
-      ref[w] = *reinterpret_cast<const float2*>(smem + w * kRingBytes + ROWS * STRIDE * 4 + r * 8);
-      mx = fmaxf(mx, ref[w].x);
+      weight[w] = *reinterpret_cast<const float*>(smem + w * kRingBytes + ROWS * STRIDE * 4 + r * 4);
+      mx = fmaxf(mx, weight[w]);
     }
     const float at = mx > -CUDART_INF_F ? mx : 0.f;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) {
+      weight[w] = exp2_fast(weight[w] - at);
+      tot += weight[w];
+    }
+    const float inv = tot == 0.f ? 0.f : 1.f / tot;
 #pragma unroll
     for (int c = 0; c < CPL; ++c) acc[c] = 0.f;
 #pragma unroll
     for (int w = 0; w < kSplitWarps; ++w) {
-      const float weight = exp2_fast(ref[w].x - at), f = weight * ref[w].y;
+      const float f = weight[w] * inv;
       const float* src = reinterpret_cast<const float*>(smem + w * kRingBytes) + r * STRIDE + lane;
-      tot += weight;
 #pragma unroll
       for (int c = 0; c < CPL; ++c) acc[c] = fmaf(f, src[32 * c], acc[c]);
     }
-    const float inv = tot == 0.f ? 0.f : 1.f / tot;
     const int s = r / p.group;
     const int64_t orow = ((int64_t)b * p.S + s) * p.Hq + kvh * p.group + r - s * p.group;
     if (p.joined) {
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) s_row[r][lane + 32 * c] = acc[c] * inv;
+      for (int c = 0; c < CPL; ++c) s_row[r][lane + 32 * c] = acc[c];
       if (lane == 0) s_sum[r] = tot == 0.f ? -CUDART_INF_F : at + log2f(tot);
     } else if (p.splits == 1) {
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) ((T*)p.out)[orow * D + lane + 32 * c] = from_f32<T>(acc[c] * inv);
+      for (int c = 0; c < CPL; ++c) ((T*)p.out)[orow * D + lane + 32 * c] = from_f32<T>(acc[c]);
     } else {
       const int64_t at_part = orow * p.splits + split;
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) p.part[at_part * D + lane + 32 * c] = acc[c] * inv;
+      for (int c = 0; c < CPL; ++c) p.part[at_part * D + lane + 32 * c] = acc[c];
       if (lane == 0) p.lse[at_part] = tot == 0.f ? -CUDART_INF_F : at + log2f(tot);
     }
   }
@@ -501,7 +512,7 @@ attention_split_kernel(const AttendParams p) {
       float sum = -CUDART_INF_F;
       if (lane < p.splits) sum = load_cluster(tc::mapa_u32(tc::smem_u32(&s_sum[r]), lane));
       const float mx = warp_max(sum), at = mx > -CUDART_INF_F ? mx : 0.f;
-      const float mine = exp2_fast(sum - at), tot = warp_sum(mine);
+      const float part = exp2_fast(sum - at), tot = warp_sum(part), mine = tot == 0.f ? 0.f : part / tot;
       float acc[CPL];
 #pragma unroll
       for (int c = 0; c < CPL; ++c) acc[c] = 0.f;
@@ -511,11 +522,10 @@ attention_split_kernel(const AttendParams p) {
 #pragma unroll
         for (int c = 0; c < CPL; ++c) acc[c] = fmaf(w, load_cluster(src + 128 * c), acc[c]);
       }
-      const float inv = tot == 0.f ? 0.f : 1.f / tot;
       const int s = r / p.group;
       const int64_t orow = ((int64_t)b * p.S + s) * p.Hq + kvh * p.group + r - s * p.group;
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) ((T*)p.out)[orow * D + lane + 32 * c] = from_f32<T>(acc[c] * inv);
+      for (int c = 0; c < CPL; ++c) ((T*)p.out)[orow * D + lane + 32 * c] = from_f32<T>(acc[c]);
     }
     tc::cluster_sync_all();                                        // nobody leaves while its rows are read
   }
@@ -860,7 +870,7 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
       // The scores of one block at a time are in registers: the second block's are read for the maximum first, and once more
       // after the first block's weights (all 128 of them would not leave the other warps enough registers).
       uint32_t a[2][32];
-      float mx = -CUDART_INF_F;
+      float top_of[2];
 #pragma unroll
       for (int h = 1; h >= 0; --h) {
 #pragma unroll
@@ -872,8 +882,9 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
 #pragma unroll
           for (int c = 0; c < 32; c += 2)
             top[(c >> 1) & 3] = max3(top[(c >> 1) & 3], __uint_as_float(a[q][c]), __uint_as_float(a[q][c + 1]));
-        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), f[h], lvs[h]));
+        top_of[h] = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), f[h], lvs[h]);
       }
+      const float mx = fmaxf(fmaxf(top_of[0], top_of[1]), -CUDART_INF_F);        // NaN counts as nothing here
       const bool move = mx > ref + kGrow || (ref == -CUDART_INF_F && mx > ref);
       if (__any_sync(0xffffffffu, move)) {                         // the reference moves, the sums so far follow
         const float alpha = move ? exp2_fast(ref - mx) : 1.f;
@@ -891,6 +902,9 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
         }
       }
       const float at = ref > -CUDART_INF_F ? ref : 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (top_of[h] > -CUDART_INF_F) lvs[h] += fmaxf(at - kFar - top_of[h], 0.f);
       float sum[2];
       // The exponentials of the two tiles take turns: at the same time they would only wait for one another and leave the
       // tensor cores idle afterwards.
@@ -944,7 +958,7 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
       tc::tc_fence_after();
     }
     const bool any = active && ok && mine && l != 0.f;
-    const float scale = any ? exp2_fast(ref - ml) / l : 0.f;
+    const float whole = ml + log2f(l), half = any ? exp2_fast(0.5f * (ref - whole)) : 0.f;
     const int64_t orow = (b * p.S + s_tok) * p.Hq + kvh * p.group + row % p.group;
 #pragma unroll 1
     for (int c = 0; c < D; c += 32) {
@@ -958,13 +972,13 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
         for (int e = 0; e < 32; e += 8) {
           float v[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) v[x] = any ? __uint_as_float(o[e + x]) * scale : 0.f;
+          for (int x = 0; x < 8; ++x) v[x] = any ? __uint_as_float(o[e + x]) * half * half : 0.f;
           if (p.splits == 1) VecIO<T, 8>::store((T*)p.out + orow * D + c + e, v);
           else VecIO<float, 8>::store(p.part + (orow * p.splits + split) * D + c + e, v);
         }
       }
     }
-    if (p.splits > 1 && row < p.rows) p.lse[orow * p.splits + split] = any ? ml + log2f(l) : -CUDART_INF_F;
+    if (p.splits > 1 && row < p.rows) p.lse[orow * p.splits + split] = any ? whole : -CUDART_INF_F;
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -972,8 +986,9 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
   if (threadIdx.x == 0 && *abort_flag) flag_status(p.status, Q3_STATUS_WAIT_TIMEOUT);
 }
 
-// out[row] = sum_i part[row, i] 2^{lse_i} / sum_i 2^{lse_i}; one warp per row, the splits' weights shared out over the
-// lanes, 32 at a time, then every lane adds up its D / 32 columns in the order of the splits.
+// out[row] = sum_i part[row, i] 2^{lse_i} / sum_i 2^{lse_i}; one warp per row, the splits' weights - divided by their sum
+// first: a sum of large rows may not be finite - shared out over the lanes, 32 at a time, then every lane adds up its D / 32
+// columns in the order of the splits.
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
 attention_merge_kernel(const float* __restrict__ part, const float* __restrict__ lse, T* __restrict__ out, int64_t rows, int splits) {
@@ -988,12 +1003,13 @@ attention_merge_kernel(const float* __restrict__ part, const float* __restrict__
   mx = warp_max(mx);
   const float ref = mx > -CUDART_INF_F ? mx : 0.f;
   float tot = 0.f, acc[CPL];
+  for (int i = lane; i < splits; i += 32) tot += exp2_fast(ls[i] - ref);
+  tot = warp_sum(tot);
 #pragma unroll
   for (int c = 0; c < CPL; ++c) acc[c] = 0.f;
   const float* src = part + row * splits * D + lane * CPL;
   for (int base = 0; base < splits; base += 32) {
-    const float mine = base + lane < splits ? exp2_fast(ls[base + lane] - ref) : 0.f;
-    tot += warp_sum(mine);
+    const float mine = base + lane < splits && tot != 0.f ? exp2_fast(ls[base + lane] - ref) / tot : 0.f;
     const int n = splits - base < 32 ? splits - base : 32;
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
@@ -1009,7 +1025,7 @@ attention_merge_kernel(const float* __restrict__ part, const float* __restrict__
   }
   T* o = out + row * D + lane * CPL;
 #pragma unroll
-  for (int c = 0; c < CPL; ++c) o[c] = from_f32<T>(tot == 0.f ? 0.f : acc[c] / tot);
+  for (int c = 0; c < CPL; ++c) o[c] = from_f32<T>(acc[c]);
 }
 
 // How a call is cut. Up to 16 rows: rows in one tile of 8 or 16, the units in `splits` pieces, for CTAs of eight warps (one per
