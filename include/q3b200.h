@@ -493,7 +493,7 @@ int q3_select_tokens(const void* logits, int64_t B, int64_t V, int64_t* ids, int
 
 /* A cache [batch, heads, capacity tokens, head_dim] of keys and values in 8 bits, for 16-bit models (dtype Q3_BF16 or
  * Q3_F16; head_dim 64 or 128). Tokens are held in blocks of 64. A complete block of one kv head stands for n * scale
- * with scale = amax / 127 over its 64 x head_dim elements (1 if all are zero) and n = round_half_even(127 x / amax) as
+ * with scale = amax / 127 over its 64 x head_dim elements (2^-126 if all are zero) and n = round_half_even(127 x / amax) as
  * int8; the incomplete last block stands for its tokens as they were given. A block of which an element is NaN or
  * infinite stands for NaN throughout. What the cache holds depends on the tokens alone, not on how appends were cut.
  * All buffers are the caller's, on one device; with blocks = ceil(capacity / 64):

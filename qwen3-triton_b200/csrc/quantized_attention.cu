@@ -66,10 +66,9 @@ template <> __device__ __forceinline__ uint32_t recent_pair<__nv_bfloat16>(uint3
   const float a = __uint_as_float(w << 16) * up, b = __uint_as_float(w & 0xffff0000u) * up;
   return pack_half(fminf(fmaxf(a, -65504.f), 65504.f), fminf(fmaxf(b, -65504.f), 65504.f));
 }
-// the power of two that takes magnitudes up to `amax` below 2^15, as far as fp32 holds it and its reciprocal (bf16 only:
-// fp16 elements stay as they are)
+// the power of two that takes magnitudes up to `amax` below 2^15, as far as fp32 holds it and its reciprocal: the largest for
+// zeros, whose weights then leave those of small values their digits (bf16 only: fp16 elements stay as they are)
 template <typename T> __device__ __forceinline__ float up_scale(float amax) {
-  if (sizeof(T) == 2 && !(amax > 0.f)) return 1.f;
   int e = 14 - ((int)(__float_as_uint(amax) >> 23) - 127);
   e = e > 126 ? 126 : (e < -126 ? -126 : e);
   return __uint_as_float((uint32_t)(e + 127) << 23);

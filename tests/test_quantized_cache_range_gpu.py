@@ -1,6 +1,6 @@
 """Attention over the 8-bit cache where the sizes of its values differ from block to block, by more than fp32's range of
-exponents if need be: blocks of any size in any order within one warp's and one CTA's share, and blocks at the ends of the
-range."""
+exponents if need be: blocks of any size in any order within one warp's and one CTA's share, blocks at the ends of the range,
+and blocks of zeros beside small values."""
 import pytest
 import torch
 
@@ -74,3 +74,13 @@ def test_value_scales_of_any_ratio_in_any_order(sizes, s, d, batch):
 def test_values_at_the_ends_of_the_range(size, s, blocks, batch):
     """All values tiny, or so large that a sum of two is not finite: in one piece, joined pieces and merged pieces."""
     attend([size] * blocks, s, 128, torch.bfloat16, batch)
+
+
+@pytest.mark.parametrize('dtype,size', [(torch.bfloat16, 1e-3), (torch.bfloat16, 1e-5), (torch.bfloat16, 1e-6), (torch.bfloat16, 1e-20),
+                                        (torch.float16, 1e-3), (torch.float16, 1e-5), (torch.float16, 1e-6)])
+@pytest.mark.parametrize('s', [1, 3, 40])
+@pytest.mark.parametrize('tail', [0, 50])
+@pytest.mark.parametrize('batch', [1, 160])
+def test_blocks_of_zeros_beside_small_values(dtype, s, size, tail, batch):
+    attend([size, 0.0, size, size, 0.0, 0.0, size], s, 64, dtype, batch, tail)
+    attend([size, 0.0, size, 0.0], s, 64, dtype, batch, tail)               # the zeros last
