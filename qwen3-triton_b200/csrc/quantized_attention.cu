@@ -60,20 +60,21 @@ template <> __device__ __forceinline__ uint32_t to_half_pair<__nv_bfloat16>(uint
 }
 // the same of recent tokens: one that `up` does not speak for, because it is not counted in, must not become infinite - its
 // weight of 0 would make NaN of it
-template <typename T> __device__ __forceinline__ uint32_t recent_pair(uint32_t w, float up);
-template <> __device__ __forceinline__ uint32_t recent_pair<__half>(uint32_t w, float) { return w; }
-template <> __device__ __forceinline__ uint32_t recent_pair<__nv_bfloat16>(uint32_t w, float up) {
-  const float a = __uint_as_float(w << 16) * up, b = __uint_as_float(w & 0xffff0000u) * up;
-  return pack_half(fminf(fmaxf(a, -65504.f), 65504.f), fminf(fmaxf(b, -65504.f), 65504.f));
+template <typename T> __device__ __forceinline__ uint32_t recent_pair(uint32_t w, float up) {
+  float a, b;
+  pair_to_f32<T>(w, a, b);
+  return pack_half(fminf(fmaxf(a * up, -65504.f), 65504.f), fminf(fmaxf(b * up, -65504.f), 65504.f));
 }
-// the power of two that takes magnitudes up to `amax` below 2^15, as far as fp32 holds it and its reciprocal: the largest for
-// zeros, whose weights then leave those of small values their digits (bf16 only: fp16 elements stay as they are)
-template <typename T> __device__ __forceinline__ float up_scale(float amax) {
+// The power of two that takes magnitudes up to `amax` below 2^15, as far as fp32 holds it and its reciprocal: the largest for
+// zeros. Recent tokens take it in both types: their weights then hold their size, as those of complete blocks hold their
+// scale, and neither takes the other's digits. Queries take it in bf16 only: fp16 is what they are to become.
+__device__ __forceinline__ float up_scale(float amax) {
   int e = 14 - ((int)(__float_as_uint(amax) >> 23) - 127);
   e = e > 126 ? 126 : (e < -126 ? -126 : e);
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
-template <> __device__ __forceinline__ float up_scale<__half>(float) { return 1.f; }
+template <typename T> __device__ __forceinline__ float query_scale(float amax) { return up_scale(amax); }
+template <> __device__ __forceinline__ float query_scale<__half>(float) { return 1.f; }
 
 // Largest magnitude of the first `live` tokens of a ring slot, by the whole CTA: where fewer tokens are counted in than the
 // slot's mark speaks for, its amax may be of others that dwarf them.
@@ -237,7 +238,7 @@ attention_split_kernel(const AttendParams p) {
       }
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const float up = up_scale<T>(amax);
+    const float up = query_scale<T>(amax);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -411,7 +412,7 @@ attention_split_kernel(const AttendParams p) {
       }
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) vw[i] = *reinterpret_cast<const uint2*>(vr + (8 * i + g) * kBlock + 16 * t + 4 * warp);
-    const float kup = up_scale<T>(mark[0].amax), vup = up_scale<T>(mark[1].amax);
+    const float kup = up_scale(mark[0].amax), vup = up_scale(mark[1].amax);
     clear_scores();
 #pragma unroll
     for (int c = 0; c < CH; ++c)
@@ -663,7 +664,7 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
     // ---------------------------------------------------------------- widen
     asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     const int tid = threadIdx.x, g = (tid >> 2) & 7, t = tid & 3, upper = tid >> 5;
-    const float lift[2] = {tail ? up_scale<T>(mark[0].amax) : 1.f, tail ? up_scale<T>(mark[1].amax) : 1.f};
+    const float lift[2] = {tail ? up_scale(mark[0].amax) : 1.f, tail ? up_scale(mark[1].amax) : 1.f};
     auto put = [&](uint32_t row_at, uint32_t x, const uint32_t (&w)[8]) {
       asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (((2 * t) ^ x) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
       asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (((2 * t + 1) ^ x) << 4)), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
@@ -804,7 +805,7 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
         for (int e = 0; e < 4; ++e)
           amax = fmaxf(amax, fmaxf(__uint_as_float(w[e] << 16 & 0x7fffffffu), __uint_as_float(w[e] & 0x7fff0000u)));
       }
-      const float up = up_scale<T>(amax);
+      const float up = query_scale<T>(amax);
       rowf = p.scale_log2 / up;
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
@@ -825,8 +826,8 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
         ks[h] = vs[h] = 1.f;
         if (blk < whole) { ks[h] = __ldg(kscale + blk); vs[h] = __ldg(vscale + blk); }
         else if (tail && blk == complete) {
-          ks[h] = mark[0].bad ? CUDART_NAN_F : 1.f / up_scale<T>(mark[0].amax);
-          vs[h] = mark[1].bad ? CUDART_NAN_F : 1.f / up_scale<T>(mark[1].amax);
+          ks[h] = mark[0].bad ? CUDART_NAN_F : 1.f / up_scale(mark[0].amax);
+          vs[h] = mark[1].bad ? CUDART_NAN_F : 1.f / up_scale(mark[1].amax);
         }
       }
     };

@@ -89,6 +89,17 @@ __device__ __forceinline__ Span span_of(int64_t b, int64_t S, int64_t capacity, 
   return s;
 }
 
+template <typename T> __device__ __forceinline__ void pair_to_f32(uint32_t w, float& a, float& b);
+template <> __device__ __forceinline__ void pair_to_f32<__nv_bfloat16>(uint32_t w, float& a, float& b) {
+  a = __uint_as_float(w << 16);
+  b = __uint_as_float(w & 0xffff0000u);
+}
+template <> __device__ __forceinline__ void pair_to_f32<__half>(uint32_t w, float& a, float& b) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  a = f.x;
+  b = f.y;
+}
+
 // two fp32 in one register pair: one instruction for both
 __device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
   uint64_t r;

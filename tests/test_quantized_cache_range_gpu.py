@@ -1,6 +1,6 @@
 """Attention over the 8-bit cache where the sizes of its values differ from block to block, by more than fp32's range of
 exponents if need be: blocks of any size in any order within one warp's and one CTA's share, blocks at the ends of the range,
-and blocks of zeros beside small values."""
+blocks of zeros beside small values, and recent tokens beside complete blocks."""
 import pytest
 import torch
 
@@ -84,3 +84,12 @@ def test_values_at_the_ends_of_the_range(size, s, blocks, batch):
 def test_blocks_of_zeros_beside_small_values(dtype, s, size, tail, batch):
     attend([size, 0.0, size, size, 0.0, 0.0, size], s, 64, dtype, batch, tail)
     attend([size, 0.0, size, 0.0], s, 64, dtype, batch, tail)               # the zeros last
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('s', [1, 3, 40])
+@pytest.mark.parametrize('size', [1.0, 1e-2, 1e-4, 1e-6])
+def test_small_values_of_complete_blocks_beside_a_heavy_recent_token(dtype, s, size):
+    """Half of the weight on a recent token: what the 64 of the block beside it hold must keep its digits."""
+    attend([size, size], s, 128, dtype, 1, 50, peak=100.0)
+    attend([size] * 6, s, 128, dtype, 1, 50, peak=300.0)
