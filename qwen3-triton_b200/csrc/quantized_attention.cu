@@ -6,9 +6,9 @@
 // scales are, and numerator and denominator keep a running reference each (m, ml). Weights are rounded to fp16 after a
 // factor of 2^15: 11 bits down to 2^-29 of the largest. Integers are exact in fp16; queries in bf16 are taken to fp16 by a
 // power of two per row, and the incomplete block's tokens by one per block. Products accumulate in fp32.
-// The denominator adds up the weights too, block by block, with vs taken out again. A block whose largest weight is below
-// 2^-kFar counts with a larger vs, such that it is 2^-kFar: in fp16 its weights are zero with either, and its share of the
-// denominator does not flush. The last factor 2^{m - ml} / sum reaches beyond fp32's exponents and is applied as two halves.
+// The denominator adds up the weights too, block by block, with vs taken out again. Where vs is below 2^-kFar of the largest so
+// far and the block's largest weight below 2^-kFar, the block counts with a larger vs, such that this weight is 2^-kFar: in fp16
+// its weights are zero with either, and its share of the denominator does not flush. The last factor 2^{m - ml} / sum reaches beyond fp32's exponents and is applied as two halves.
 #include "quantized_cache.cuh"
 #include "tcgen05.cuh"
 #include <math_constants.h>
@@ -270,12 +270,15 @@ attention_split_kernel(const AttendParams p) {
   float sc[NT][4][4];
   uint32_t pf[NT][8];
   bool ok = true;
+  float top_lvs = -CUDART_INF_F;                                   // of the blocks so far
 
   // scores of 16 * IT tokens from `token` on -> weights in pf; o rescaled
   auto softmax = [&](auto it_count, int token, float ks, float vs) {
     constexpr int IT = decltype(it_count)::value;
     const float lvs = log2f(vs);
     const bool masked = token + 16 * IT > unmasked;
+    top_lvs = fmaxf(top_lvs, lvs);
+    const bool far = lvs < top_lvs - kFar;                         // only then can weights flush that count
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float alpha[2], ref[2];
@@ -298,7 +301,12 @@ attention_split_kernel(const AttendParams p) {
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         const float nm = fmaxf(m[nt][e], mx);
         ref[e] = nm > -CUDART_INF_F ? nm : 0.f;
-        const float far = mx > -CUDART_INF_F ? fmaxf(ref[e] - kFar - mx, 0.f) : 0.f;     // what log2 vs is raised by
+        float base = ref[e] - 15.f, d = ref[e] - lvs;
+        if (far && mx > -CUDART_INF_F) {
+          const float raise = fmaxf(ref[e] - kFar - mx, 0.f);      // of log2 vs
+          base -= raise;
+          d -= raise;
+        }
         alpha[e] = exp2_fast(m[nt][e] - ref[e]);
         m[nt][e] = nm;
         float sum = 0.f;
@@ -306,12 +314,12 @@ attention_split_kernel(const AttendParams p) {
         for (int it = 0; it < IT; ++it)
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
-            const float w = exp2_fast(sc[nt][it][2 * hf + e] - (ref[e] - 15.f - far));
+            const float w = exp2_fast(sc[nt][it][2 * hf + e] - base);
             sc[nt][it][2 * hf + e] = w;
             sum += w;
           }
         if (ahead > 0) {                                           // the same in all lanes of a row
-          const float d = ref[e] - lvs - far, nml = fmaxf(ml[nt][e], d);
+          const float nml = fmaxf(ml[nt][e], d);
           l[nt][e] = l[nt][e] * exp2_fast(ml[nt][e] - nml) + sum * exp2_fast(d - nml);
           ml[nt][e] = nml;
         }
@@ -833,7 +841,7 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
     };
     // without the recent tokens there is nothing from the incomplete block on
     if (!tail && visible > complete * kBlock) visible = complete * kBlock;
-    float ks[2], vs[2];
+    float ks[2], vs[2], top_lvs = -CUDART_INF_F;
     if (active) scales(t0, ks, vs);
     for (int j = 0; j < n && ok; ++j) {
       const int ahead = visible - (t0 + j) * 128;
@@ -845,6 +853,8 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
         f[h] = ks[h] * rowf;
         if (f[h] < 1e-37f || limit <= h * 64) f[h] = 1e-37f;       // -inf times it stays -inf; NaN stays where the row sees it
       }
+      top_lvs = fmaxf(top_lvs, fmaxf(lvs[0], lvs[1]));
+      const bool far = fminf(lvs[0], lvs[1]) < top_lvs - kFar;     // only then can weights flush that count
       if (j + 1 < n) scales(t0 + j + 1, ks, vs);
       ok = __all_sync(0xffffffffu, tc::mbar_wait(s_full(i), j & 1u, abort_flag));
       if (!ok) break;
@@ -901,10 +911,12 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
           }
         }
       }
-      const float at = ref > -CUDART_INF_F ? ref : 0.f;
+      if (far) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (top_of[h] > -CUDART_INF_F) lvs[h] += fmaxf(at - kFar - top_of[h], 0.f);
+        for (int h = 0; h < 2; ++h)
+          if (top_of[h] > -CUDART_INF_F) lvs[h] += fmaxf(ref - kFar - top_of[h], 0.f);
+      }
+      const float at = ref > -CUDART_INF_F ? ref : 0.f;
       float sum[2];
       // The exponentials of the two tiles take turns: at the same time they would only wait for one another and leave the
       // tensor cores idle afterwards.
