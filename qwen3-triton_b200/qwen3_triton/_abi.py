@@ -16,6 +16,10 @@ import torch
 Q3_F32, Q3_BF16, Q3_F16 = 0, 1, 2
 STATUS_ID_RANGE, STATUS_LABEL_RANGE, STATUS_WAIT_TIMEOUT, STATUS_EMPTY_TARGETS = 1, 2, 4, 8
 STATUS_CACHE_RANGE, STATUS_CACHE_RECENT = 16, 32
+_STATUS_TEXT = {STATUS_ID_RANGE: "embedding id out of range", STATUS_LABEL_RANGE: "label out of range",
+                STATUS_WAIT_TIMEOUT: "kernel wait timed out", STATUS_EMPTY_TARGETS: "no valid cross-entropy target",
+                STATUS_CACHE_RANGE: "8-bit cache: tokens outside the capacity",
+                STATUS_CACHE_RECENT: "8-bit cache: earlier tokens of an incomplete block not held"}
 
 _DTYPES = {torch.float32: Q3_F32, torch.bfloat16: Q3_BF16, torch.float16: Q3_F16}
 FLOAT_DTYPES = tuple(_DTYPES)
@@ -213,6 +217,6 @@ def read_status(device=None, *, clear=True) -> int:
 def raise_on_status(device=None) -> None:
     value = read_status(device)
     if value:
-        names = [n for bit, n in ((1, "embedding id out of range"), (2, "label out of range"),
-                                  (4, "kernel wait timed out"), (8, "no valid cross-entropy target")) if value & bit]
-        raise Q3Error("device status: " + ", ".join(names))
+        names = [n for bit, n in _STATUS_TEXT.items() if value & bit]
+        rest = value & ~sum(_STATUS_TEXT)
+        raise Q3Error("device status: " + ", ".join(names + ([f"unknown bits {rest:#x}"] if rest else [])))
