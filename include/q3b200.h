@@ -521,8 +521,10 @@ typedef struct q3_quantized_cache {
 
 /* Append k, v [B,S,H,D] (token-major, as q3_kv_append takes them) after `start` tokens. A start inside a block needs that
  * block's earlier tokens among the recent ones: a sequence may go back (start below its length) to any token of its last
- * two blocks, or to any multiple of 64; otherwise Q3_STATUS_CACHE_RECENT is set and that sequence must not be used. At most
- * 4194176 new tokens in a call. */
+ * two blocks, or to any multiple of 64; otherwise Q3_STATUS_CACHE_RECENT is set. The sequence then stays as it was if the call
+ * would have left that block incomplete. If it completes the block, the block holds other tokens in the place of the missing ones,
+ * and every later call that reaches it sets the bit again, until it is written anew from its first token. At most 4194176 new
+ * tokens in a call. */
 int q3_qcache_append(const q3_quantized_cache* cache, const void* k, const void* v, int64_t S, int64_t start,
                      const int64_t* starts, const int64_t* counts, int* status, q3_stream_t stream);
 

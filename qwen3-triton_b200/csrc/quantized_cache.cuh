@@ -27,8 +27,12 @@ __host__ __device__ constexpr int value_offset(int token, int dim) { return dim 
 // What the ring holds: slot (block % 2) of a (sequence, head) holds the first `fill` tokens of `block`. `bad` is 0, or 1 +
 // the first of them that had a NaN or an infinity (those are stored as 0); `amax` is at least their largest magnitude, and at
 // most 2^10 times as much (attention takes them to fp16 by a power of two). One mark for the keys and one for the values.
+// `torn`, the same in all marks of a (sequence, head): 0, or 1 + the first complete block whose earlier tokens were not held when
+// it was completed; whoever reads it or what follows is told so, until it is written anew from its first token.
 struct Mark {
-  int block, fill, bad;
+  int block;
+  short fill, bad;
+  int torn;
   float amax;
 };
 

@@ -1,0 +1,115 @@
+"""What the 8-bit cache promises around the edges of its contract: appends that it refuses, stepping back more than once, padded
+calls at the end of the cache, caches much longer than their sequences, and where each byte lies."""
+import pytest
+import torch
+
+from helpers import randn
+from oracle import quantized as OQ
+from test_quantized_cache_gpu import expect_attention, expect_read, lengths, make, tokens
+
+pytestmark = pytest.mark.gpu
+
+
+def part(x, first, last):
+    return x[:, first:last].contiguous().cuda()
+
+
+def reported():
+    """Whether the status names missing tokens, and nothing else."""
+    from qwen3_triton import _abi
+    status = _abi.read_status()
+    assert status in (0, _abi.STATUS_CACHE_RECENT)
+    return status != 0
+
+
+def test_a_refused_append_to_an_incomplete_block_leaves_the_sequence_alone():
+    """A gap: the block's earlier tokens are not all there. What was held stays; the length that the call was to reach is reported."""
+    from qwen3_triton.inference import quantized as Q
+    dtype, h, d, t = torch.bfloat16, 2, 64, 400
+    k, v = tokens(2, t, h, d, dtype, 21)
+    cache = make(2, h, t, d, dtype)
+    Q.append(part(k, 0, 300), part(v, 0, 300), cache, 0)
+    buffers = (cache.keys, cache.values, cache.key_scales, cache.value_scales, cache.recent_keys, cache.recent_values, cache.marks)
+    before = [x.clone() for x in buffers]
+    for start, n in [(310, 1), (301, 19), (100, 3), (330, 50)]:              # in the block, to its end, an older block, the next one
+        n = min(n, 63 - start % 64)
+        Q.append(part(k, start, start + n), part(v, start, start + n), cache, start)
+        assert reported()
+        assert all(torch.equal(x, y) for x, y in zip(before, buffers)), start
+        Q.read(cache, start + n)
+        assert reported()
+        for s in (1, 40):
+            Q.attention(randn((2, s, 4, d), 1, dtype).cuda(), cache, start + n - s)
+            assert reported()
+    for i in range(2):
+        expect_read(Q.read(cache, 300)[0][i], k[i], 300)
+    Q.append(part(k, 300, 400), part(v, 300, 400), cache, 300)
+    for i in range(2):
+        expect_read(Q.read(cache, 400)[1][i], v[i], 400)
+    assert not reported()
+
+
+@pytest.mark.parametrize('start,n', [(100, 28), (100, 29), (100, 92), (100, 93), (100, 200), (70, 250)])
+@pytest.mark.parametrize('ragged', [False, True])
+def test_a_refused_append_that_completes_its_block_is_reported_until_it_is_written_anew(start, n, ragged):
+    from qwen3_triton.inference import quantized as Q
+    dtype, h, d, t = torch.float16, 1, 128, 700
+    k, v = tokens(2, t, h, d, dtype, 23)
+    cache = make(2, h, t, d, dtype)
+    Q.append(part(k, 0, 600), part(v, 0, 600), cache, 0)
+    end = start + n
+    where = lengths(start, start) if ragged else start
+    Q.append(part(k, start, end), part(v, start, end), cache, where)         # blocks 8 and 9 are held, not block 1
+    assert reported()
+
+    def all_report():
+        seen = []
+        for s in (1, 40):
+            Q.attention(randn((2, s, 2, d), 1, dtype).cuda(), cache, end - s)
+            seen.append(reported())
+        Q.read(cache, end)
+        seen.append(reported())
+        Q.read(cache, end, 64, 5)
+        seen.append(reported())
+        return seen
+
+    assert all(all_report())
+    Q.append(part(k, end, end + 70), part(v, end, end + 70), cache, end)     # more tokens do not make it right
+    assert reported()
+    end += 70
+    assert all(all_report())
+    Q.append(part(k, 110, 120), part(v, 110, 120), cache, 110)               # nor does another step back into the block
+    assert reported()
+    Q.read(cache, 64)                                                        # what lies before it is untouched
+    assert not reported()
+    expect_read(Q.read(cache, 64)[1][0], v[0], 64)
+    Q.attention(randn((2, 1, 2, d), 1, dtype).cuda(), cache, 63)
+    assert not reported()
+    Q.append(part(k, 64, end), part(v, 64, end), cache, 64)                  # the block anew
+    assert not any(all_report())
+    for i in range(2):
+        expect_read(Q.read(cache, end)[0][i], k[i], end)
+        expect_read(Q.read(cache, end)[1][i], v[i], end)
+    Q.append(part(k, end, end + 5), part(v, end, end + 5), cache, end)
+    assert not reported()
+    expect_read(Q.read(cache, end + 5)[1][1], v[1], end + 5)
+
+
+def test_a_new_sequence_in_the_place_of_a_refused_one():
+    from qwen3_triton.inference import quantized as Q
+    dtype, h, d, t = torch.bfloat16, 1, 64, 400
+    k, v = tokens(1, t, h, d, dtype, 25)
+    for n in (1, 64, 65, 300):
+        cache = make(1, h, t, d, dtype)
+        Q.append(part(k, 0, 300), part(v, 0, 300), cache, 0)
+        Q.append(part(k, 100, 300), part(v, 100, 300), cache, 100)
+        assert reported()
+        Q.append(part(k, 0, n), part(v, 0, n), cache, 0)
+        assert not reported()
+        q = randn((1, 1, 2, d), 26, dtype)
+        expect_attention(Q.attention(q.cuda(), cache, n - 1)[0], q[0], k[0, :n], v[0, :n], n - 1, dtype)
+        expect_read(Q.read(cache, n)[0][0], k[0], n)
+        assert not reported()
+        Q.append(part(k, n, n + 70), part(v, n, n + 70), cache, n)
+        expect_read(Q.read(cache, n + 70)[0][0], k[0], n + 70)
+        assert not reported()
