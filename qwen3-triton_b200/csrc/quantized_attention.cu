@@ -1141,11 +1141,11 @@ using namespace q3;
 // host checks shared by the call and its workspace query, and how the call is cut; `start` < 0: lengths on the device
 static int plan_checked(const q3_quantized_cache* cache, int64_t S, int64_t Hq, int64_t start, qc::Plan* plan, int64_t* bytes) {
   if (int rc = qc::check_cache(cache); rc != Q3_OK) return rc;
-  if (S < 1 || S > cache->capacity || Hq < 1 || Hq % cache->heads || Hq > (int64_t)1 << 16 || start > cache->capacity - S)
+  if (S < 1 || S > cache->capacity || Hq < 1 || Hq % cache->heads || Hq > (int64_t)1 << 16 || start > cache->capacity)
     return Q3_ERR_SHAPE;
   const int64_t bh = cache->batch * cache->heads, rows = S * (Hq / cache->heads);
   if (rows > (int64_t)1 << 30) return Q3_ERR_SHAPE;
-  *plan = qc::plan_attention(bh, rows, start < 0 ? cache->capacity : start + S);
+  *plan = qc::plan_attention(bh, rows, start < 0 || start > cache->capacity - S ? cache->capacity : start + S);
   if (bh * plan->tiles > 0x7fffffff / plan->splits) return Q3_ERR_SHAPE;
   *bytes = plan->splits == 1 || plan->joined ? 0 : cache->batch * S * Hq * plan->splits * (cache->head_dim + 1) * 4;
   return Q3_OK;
@@ -1162,7 +1162,7 @@ extern "C" int q3_qcache_attention(const q3_quantized_cache* cache, const void* 
                                    const int64_t* counts, double scale, int* status, q3_stream_t stream) {
   if (int rc = qc::check_cache(cache); rc != Q3_OK) return rc;
   if (!q || !out || !(scale > 0)) return Q3_ERR_ARG;
-  if (!starts && start < 0) return Q3_ERR_SHAPE;
+  if (!starts && (start < 0 || start > cache->capacity - (counts ? 0 : S))) return Q3_ERR_SHAPE;
   qc::Plan pl;
   int64_t need = 0;
   if (int rc = plan_checked(cache, S, Hq, starts ? -1 : start, &pl, &need); rc != Q3_OK) return rc;

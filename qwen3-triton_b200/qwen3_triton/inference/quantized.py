@@ -7,8 +7,9 @@ given. What a cache holds therefore depends on its tokens alone, not on how they
 an element is NaN or infinite reads back as NaN.
 
 Lengths are Python ints (the same for every sequence) or int64 CUDA tensors [B], which the kernels read when they run:
-a step captured into a CUDA graph follows them. Ints are checked here; what a tensor holds is checked on the device,
-where a violation leaves the sequence alone and shows in the status word (_abi.raise_on_status).
+a step captured into a CUDA graph follows them. Ints are checked here; what a tensor holds (with `count` also whether
+start and count together fit) is checked on the device, where a violation leaves the sequence alone and shows in the
+status word (_abi.raise_on_status).
 """
 import ctypes
 import operator
@@ -112,7 +113,7 @@ def append(k, v, cache, start, count=None):
     if _elsewhere(cache):
         with torch.cuda.device(cache.device):
             return append(k, v, cache, start, count)
-    start, starts = _length(start, cache, cache.capacity - s, 'start')
+    start, starts = _length(start, cache, cache.capacity - (s if count is None else 0), 'start')
     counts = _counts(count, cache)
     _launch(_abi.lib().q3_qcache_append, cache, k.data_ptr(), v.data_ptr(), s, start, _abi.ptr(starts), _abi.ptr(counts))
 
@@ -152,7 +153,7 @@ def attention(q, cache, start, count=None):
     if _elsewhere(cache):
         with torch.cuda.device(cache.device):
             return attention(q, cache, start, count)
-    start, starts = _length(start, cache, cache.capacity - s, 'start')
+    start, starts = _length(start, cache, cache.capacity - (s if count is None else 0), 'start')
     counts = _counts(count, cache)
     out = torch.empty_like(q)
     lib = _abi.lib()

@@ -113,3 +113,34 @@ def test_a_new_sequence_in_the_place_of_a_refused_one():
         Q.append(part(k, n, n + 70), part(v, n, n + 70), cache, n)
         expect_read(Q.read(cache, n + 70)[0][0], k[0], n + 70)
         assert not reported()
+
+
+@pytest.mark.parametrize('s', [3, 50])
+@pytest.mark.parametrize('where', ['host', 'device'])
+def test_padding_may_reach_beyond_the_capacity(s, where):
+    """The last chunk of a sequence, padded to the size of the others: its real tokens fit, its padding does not."""
+    from qwen3_triton import _abi
+    from qwen3_triton.inference import quantized as Q
+    dtype, b, h, hq, d, cap = torch.bfloat16, 2, 2, 4, 64, 150
+    k, v = tokens(b, cap + s, h, d, dtype, 31)
+    q = randn((b, s, hq, d), 32, dtype)
+    start, counts = cap - 2, (2, 1)
+    cache = make(b, h, cap, d, dtype)
+    Q.append(part(k, 0, start), part(v, 0, start), cache, 0)
+    at = lengths(start, start) if where == 'device' else start
+    Q.append(part(k, start, start + s), part(v, start, start + s), cache, at, lengths(*counts))
+    out = Q.attention(q.cuda(), cache, at, lengths(*counts))
+    for i, n in enumerate(counts):
+        expect_attention(out[i, :n], q[i, :n], k[i, :start + n], v[i, :start + n], start, dtype)
+        assert not out[i, n:].any()
+        expect_read(Q.read(cache, lengths(*(start + c for c in counts)), 0, cap)[0][i], k[i], start + n)
+    Q.append(part(k, 0, s), part(v, 0, s), cache, cap, lengths(0, 0))         # a full cache, and nothing new
+    assert not Q.attention(q.cuda(), cache, cap, lengths(0, 0)).any()
+    assert _abi.read_status() == 0
+    Q.append(part(k, 0, s), part(v, 0, s), cache, cap - 1, lengths(1, 2))     # the second one does not fit
+    assert _abi.read_status() == _abi.STATUS_CACHE_RANGE
+    with pytest.raises(ValueError):
+        Q.append(part(k, 0, s), part(v, 0, s), cache, cap + 1, lengths(0, 0))
+    for call in (lambda: Q.append(part(k, 0, s), part(v, 0, s), cache, cap - s + 1), lambda: Q.attention(q.cuda(), cache, cap - s + 1)):
+        with pytest.raises(ValueError):
+            call()
