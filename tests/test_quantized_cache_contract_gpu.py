@@ -144,3 +144,30 @@ def test_padding_may_reach_beyond_the_capacity(s, where):
     for call in (lambda: Q.append(part(k, 0, s), part(v, 0, s), cache, cap - s + 1), lambda: Q.attention(q.cuda(), cache, cap - s + 1)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('total', [100, 128, 150, 192, 200, 333, 340])
+def test_the_recent_tokens_do_not_depend_on_the_cuts(dtype, total):
+    """The last 128 tokens as given, one slot for each, whatever the calls were: token by token, at once, and pieces that start and
+    end in the same and in different slots, before and behind one another."""
+    from qwen3_triton.inference import quantized as Q
+    h, d = 2, 64
+    k, v = tokens(1, total, h, d, dtype, 40 + total)
+    k[0, total - 70, 0, 5], v[0, total - 3, 1, 7] = float('nan'), float('inf')               # held as 0, with a mark
+    pieces = [[total], [1] * total, [50, total - 50], [30, 40, total - 70], [10, total - 30, 20], [60, total - 64, 4]]
+    want = [torch.zeros(1, h, 2, 64 * d, dtype=dtype), torch.zeros(1, h, 2, 64 * d, dtype=dtype)]
+    for t in range(max(0, total - 128), total):
+        row = t % 64
+        key = [((row // 8) * (d // 64) + x // 64) * 512 + (row % 8) * 64 + x % 64 for x in range(d)]
+        value = [x * 64 + ((row // 2) % 4) * 16 + (row // 8) * 2 + row % 2 for x in range(d)]
+        for buffer, x, places in ((want[0], k, key), (want[1], v, value)):
+            buffer[0, :, t // 64 % 2, places] = torch.where(torch.isfinite(x[0, t]), x[0, t], torch.zeros_like(x[0, t]))
+    for cut in pieces:
+        cache, at = make(1, h, total, d, dtype), 0
+        for n in cut:
+            Q.append(part(k, at, at + n), part(v, at, at + n), cache, at)
+            at += n
+        assert at == total
+        assert torch.equal(cache.recent_keys.cpu(), want[0]) and torch.equal(cache.recent_values.cpu(), want[1]), cut
+    assert not reported()
