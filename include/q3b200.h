@@ -520,8 +520,9 @@ typedef struct q3_quantized_cache {
 } q3_quantized_cache;
 
 /* Append k, v [B,S,H,D] (token-major, as q3_kv_append takes them) after `start` tokens. A start inside a block needs that
- * block's earlier tokens among the recent ones: a sequence may go back (start below its length) to any token of its last
- * two blocks, or to any multiple of 64; otherwise Q3_STATUS_CACHE_RECENT is set. The sequence then stays as it was if the call
+ * block's earlier tokens among the recent ones: a sequence may go back (start below its length) to any multiple of 64, or to any
+ * token of its last two blocks - but once it has gone back to an earlier block, only of that one, until it begins the next;
+ * otherwise Q3_STATUS_CACHE_RECENT is set. The sequence then stays as it was if the call
  * would have left that block incomplete. If it completes the block, the block holds other tokens in the place of the missing ones,
  * and every later call that reaches it sets the bit again, until it is written anew from its first token. At most 4194176 new
  * tokens in a call. */

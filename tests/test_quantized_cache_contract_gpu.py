@@ -171,3 +171,59 @@ def test_the_recent_tokens_do_not_depend_on_the_cuts(dtype, total):
         assert at == total
         assert torch.equal(cache.recent_keys.cpu(), want[0]) and torch.equal(cache.recent_values.cpu(), want[1]), cut
     assert not reported()
+
+
+def test_steps_back_in_a_row():
+    """What a sequence may go back to after it has gone back: the block it is in, and the one before only if it came from there."""
+    from qwen3_triton.inference import quantized as Q
+    dtype, h, d, t = torch.bfloat16, 2, 64, 400
+
+    def check(steps, refused=()):
+        cache, now = make(1, h, t, d, dtype), [torch.zeros(1, t, h, d, dtype=dtype) for _ in range(2)]
+        for i, (start, n) in enumerate(steps):
+            k, v = tokens(1, n, h, d, dtype, 60 + i)
+            Q.append(k.cuda(), v.cuda(), cache, start)
+            assert reported() == (i in refused), (steps, i)
+            if i in refused:
+                return
+            for x, new in zip(now, (k, v)):
+                x[:, start:start + n] = new
+            end = start + n
+            expect_read(Q.read(cache, end)[0][0], now[0][0], end)
+            expect_read(Q.read(cache, end)[1][0], now[1][0], end)
+            for s in (1, min(end, 30)):
+                q = randn((1, s, 4, d), 90 + i, dtype)
+                expect_attention(Q.attention(q.cuda(), cache, end - s)[0], q[0], now[0][0, :end], now[1][0, :end], end - s, dtype)
+            assert not reported(), (steps, i)
+
+    check([(0, 200), (195, 3), (193, 1), (150, 2), (140, 5)])            # down within blocks 3 and 2
+    check([(0, 200), (130, 3), (131, 80), (190, 1)])                     # back to block 2, on into block 3: both are held again
+    check([(0, 200), (130, 3), (100, 1)], refused=(2,))                  # block 1 was not held any more
+    check([(0, 200), (128, 3), (100, 1)], refused=(2,))
+    check([(0, 200), (64, 10), (30, 1)], refused=(2,))                   # nor block 0
+    check([(0, 200), (64, 10), (70, 60), (100, 3)])                      # blocks 1 and 2
+    check([(0, 200), (64, 10), (0, 30), (20, 100), (64, 1), (10, 3)])    # 64 lies in block 1, the last one: 0 stays held
+    check([(0, 200), (64, 10), (0, 30), (20, 100), (10, 3), (12, 60), (71, 1), (64, 3), (40, 90)])
+    check([(0, 128), (127, 1), (64, 64), (127, 1), (128, 1), (100, 1)])  # ends and starts on the boundaries
+
+
+@pytest.mark.parametrize('d', [64, 128])
+def test_where_each_byte_lies(d):
+    """The order of csrc/quantized_cache.cuh on real buffers: integers that are their own quantised form (largest magnitude 127)."""
+    from qwen3_triton.inference import quantized as Q
+    g = torch.Generator().manual_seed(3)
+    b, h, t = 2, 2, 150
+    k, v = (torch.randint(-126, 127, (b, t, h, d), generator=g) for _ in range(2))
+    for x in (k, v):
+        x[:, 5::64, :, 3] = 127
+    cache = make(b, h, t, d, torch.bfloat16)
+    Q.append(k.bfloat16().cuda(), v.bfloat16().cuda(), cache, 0)
+    row, dim = torch.arange(64)[:, None], torch.arange(d)[None]
+    key = (row // 8 * (d // 64) + dim // 64) * 512 + row % 8 * 64 + dim % 64
+    value = dim * 64 + row // 2 % 4 * 16 + row // 8 * 2 + row % 2
+    for got, scales, x, place in ((cache.keys, cache.key_scales, k, key), (cache.values, cache.value_scales, v, value)):
+        blocks = x[:, :128].transpose(1, 2).reshape(b, h, 2, 64, d)
+        want = torch.empty(b, h, 2, 64 * d, dtype=torch.uint8)
+        want[..., place.reshape(-1)] = (blocks + 128).to(torch.uint8).reshape(b, h, 2, 64 * d)
+        assert torch.equal(got[:, :, :2].cpu(), want)
+        assert torch.equal(scales[:, :, :2].cpu(), torch.ones(b, h, 2))
