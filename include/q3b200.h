@@ -53,7 +53,7 @@ enum {
   Q3_STATUS_WAIT_TIMEOUT = 4,/* a bounded barrier wait inside a kernel gave up */
   Q3_STATUS_EMPTY_TARGETS = 8,/* cross-entropy saw no valid target */
   Q3_STATUS_CACHE_RANGE = 16, /* 8-bit cache: tokens of a sequence outside the capacity */
-  Q3_STATUS_CACHE_RECENT = 32 /* 8-bit cache: earlier tokens of an incomplete block are not (or no longer) held */
+  Q3_STATUS_CACHE_RECENT = 32 /* 8-bit cache: earlier tokens are not (or, of an incomplete block, no longer) held */
 };
 
 int q3_abi_version(void);
@@ -522,15 +522,16 @@ typedef struct q3_quantized_cache {
 /* Append k, v [B,S,H,D] (token-major, as q3_kv_append takes them) after `start` tokens. A start inside a block needs that
  * block's earlier tokens among the recent ones: a sequence may go back (start below its length) to any multiple of 64, or to any
  * token of its last two blocks - but once it has gone back to an earlier block, only of that one, until it begins the next;
- * otherwise Q3_STATUS_CACHE_RECENT is set. The sequence then stays as it was if the call
- * would have left that block incomplete. If it completes the block, the block holds other tokens in the place of the missing ones,
- * and every later call that reaches it sets the bit again, until it is written anew from its first token. At most 4194176 new
- * tokens in a call. */
+ * otherwise Q3_STATUS_CACHE_RECENT is set, as it is for a start beyond the length. The sequence then stays as it was if the call
+ * leaves its first block incomplete. If it completes that block, other tokens stand in the place of the missing ones, and every
+ * later call that reaches a block without its own sets the bit again, until that is written anew. At most 4194176 new tokens in a
+ * call. */
 int q3_qcache_append(const q3_quantized_cache* cache, const void* k, const void* v, int64_t S, int64_t start,
                      const int64_t* starts, const int64_t* counts, int* status, q3_stream_t stream);
 
 /* k, v [B,H,tokens,D] (dtype) = the values of tokens first .. first + tokens - 1 of sequences that hold `length` tokens
- * (lengths[b], firsts[b] where those are given); rows at or past the length are zero. tokens <= 4194176. */
+ * (lengths[b], firsts[b] where those are given); rows at or past the length are zero. A length beyond the tokens that were
+ * appended sets Q3_STATUS_CACHE_RECENT, in attention too. tokens <= 4194176. */
 int q3_qcache_read(const q3_quantized_cache* cache, void* k, void* v, int64_t tokens, int64_t length,
                    const int64_t* lengths, int64_t first, const int64_t* firsts, int* status, q3_stream_t stream);
 

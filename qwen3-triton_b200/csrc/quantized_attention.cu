@@ -187,8 +187,8 @@ attention_split_kernel(const AttendParams p) {
   const float* vscale = p.c.scales[1] + (int64_t)bh * p.c.blocks;
   float ks = 0.f, vs = 1.f;
   if (mine > 0) { ks = kscale[first]; vs = vscale[first]; }
-  int torn = 0;
-  if (threadIdx.x == 0) torn = p.c.marks[bh * 4].torn;
+  Mark both[2] = {};                                               // of the keys, thread 0
+  if (threadIdx.x == 0) { both[0] = p.c.marks[bh * 4]; both[1] = p.c.marks[bh * 4 + 1]; }
   Mark mark[2];
   if (tail) {
     mark[0] = p.c.marks[(bh * 2 + 0) * 2 + (complete & 1)];
@@ -213,7 +213,7 @@ attention_split_kernel(const AttendParams p) {
   }
   __syncthreads();                                                 // abort_flag
   if (!fits && threadIdx.x == 0) flag_status(p.status, Q3_STATUS_CACHE_RANGE);
-  if (torn > 0 && (torn - 1) * kBlock < seen) flag_status(p.status, Q3_STATUS_CACHE_RECENT);       // thread 0
+  if (threadIdx.x == 0 && !held_whole(both, seen)) flag_status(p.status, Q3_STATUS_CACHE_RECENT);
   if (tail) {
     const int need = end - complete * kBlock;
     if (mark[0].block != complete || mark[0].fill < need || mark[1].block != complete || mark[1].fill < need) {
@@ -633,6 +633,8 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
   }
   const int start = (int)sp.start, end = (int)(sp.start + sp.count);           // a cache has at most 2^30 tokens
   const int complete = end / kBlock;
+  if (blockIdx.x < bhs && split == 0 && threadIdx.x == 0 && sp.count > 0 && !held_whole(p.c.marks + bh * 4, end))
+    flag_status(p.status, Q3_STATUS_CACHE_RECENT);
   const int row0 = tile * kPromptRows;
   const int real = (int)sp.count * p.group - row0;                 // rows of this CTA that are not padding
   const int here = real < kPromptRows ? real : kPromptRows;
@@ -642,8 +644,6 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
   const bool two = here > 128;
   const int wanted = (seen + kBlock - 1) / kBlock;                 // blocks
   const int whole = complete < wanted ? complete : wanted;         // of them, in 8 bits
-  int torn = 0;
-  if (threadIdx.x == 0) torn = p.c.marks[bh * 4].torn;
   Mark mark[2];
   mark[0].block = -1;
   if (wanted > complete) {
@@ -1001,7 +1001,6 @@ attention_prompt_kernel(const AttendParams p, const uint32_t idesc_qk, const uin
   __syncthreads();
   if (warp == 12) { tc::tc_fence_after(); tc::tmem_dealloc(tmem, 512); }
   if (threadIdx.x == 0 && *abort_flag) flag_status(p.status, Q3_STATUS_WAIT_TIMEOUT);
-  if (torn > 0 && (torn - 1) * kBlock < seen) flag_status(p.status, Q3_STATUS_CACHE_RECENT);       // thread 0
 }
 
 // out[row] = sum_i part[row, i] 2^{lse_i} / sum_i 2^{lse_i}; one warp per row, the splits' weights - divided by their sum

@@ -26,9 +26,10 @@ __host__ __device__ constexpr int value_offset(int token, int dim) { return dim 
 
 // What the ring holds: slot (block % 2) of a (sequence, head) holds the first `fill` tokens of `block`. `bad` is 0, or 1 +
 // the first of them that had a NaN or an infinity (those are stored as 0); `amax` is at least their largest magnitude, and at
-// most 2^10 times as much (attention takes them to fp16 by a power of two). One mark for the keys and one for the values.
-// `torn`, the same in all marks of a (sequence, head): 0, or 1 + the first complete block whose earlier tokens were not held when
-// it was completed; whoever reads it or what follows is told so, until it is written anew from its first token.
+// most 2^10 times as much (attention takes them to fp16 by a power of two). One mark for the keys and one for the values. A
+// block that was completed without its earlier tokens has -fill: its length counts, its tokens cannot be relied on.
+// `torn`, the same in all marks of a (sequence, head): 0, or 1 + the first complete block of which tokens were missing when it, or
+// a later one, was completed; whoever reads it or what follows is told so, until it is written anew from its first token.
 struct Mark {
   int block;
   short fill, bad;
@@ -102,6 +103,17 @@ template <> __device__ __forceinline__ void pair_to_f32<__half>(uint32_t w, floa
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
   a = f.x;
   b = f.y;
+}
+
+// Tokens that the two marks of a (sequence, head) speak for: its length after the last append.
+__device__ __forceinline__ int held_tokens(const Mark& a, const Mark& b) {
+  return max(a.block < 0 ? 0 : a.block * kBlock + abs(a.fill), b.block < 0 ? 0 : b.block * kBlock + abs(b.fill));
+}
+// Whether the first `tokens` tokens are held, none of their blocks torn. (That the incomplete block of a shorter length is
+// still among the recent ones is another question.)
+__device__ __forceinline__ bool held_whole(const Mark* marks, int tokens) {
+  const Mark a = marks[0], b = marks[1];
+  return tokens <= held_tokens(a, b) && (a.torn == 0 || tokens <= (a.torn - 1) * kBlock);
 }
 
 // two fp32 in one register pair: one instruction for both

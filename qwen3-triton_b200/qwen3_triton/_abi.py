@@ -19,7 +19,7 @@ STATUS_CACHE_RANGE, STATUS_CACHE_RECENT = 16, 32
 _STATUS_TEXT = {STATUS_ID_RANGE: "embedding id out of range", STATUS_LABEL_RANGE: "label out of range",
                 STATUS_WAIT_TIMEOUT: "kernel wait timed out", STATUS_EMPTY_TARGETS: "no valid cross-entropy target",
                 STATUS_CACHE_RANGE: "8-bit cache: tokens outside the capacity",
-                STATUS_CACHE_RECENT: "8-bit cache: earlier tokens of an incomplete block not held"}
+                STATUS_CACHE_RECENT: "8-bit cache: earlier tokens not held"}
 
 _DTYPES = {torch.float32: Q3_F32, torch.bfloat16: Q3_BF16, torch.float16: Q3_F16}
 FLOAT_DTYPES = tuple(_DTYPES)

@@ -99,10 +99,10 @@ def append(k, v, cache, start, count=None):
     """Write the new k, v [B,S,H,D] into the cache after `start` tokens of each sequence. With `count` (int64 [B]) only
     the first count[b] of the S tokens are real; the rest is padding. A sequence may go back, by a `start` below its
     length, to any multiple of 64 or to any token of its last two blocks (once it has gone back to an earlier block, only of
-    that one, until it begins the next). Any other start inside a block (tokens are missing or no longer held as given)
-    shows in _abi.raise_on_status: the sequence stays as it was if the block would have stayed incomplete; else the block
-    holds other tokens in their place, and every call that reaches it reports so, until it is written anew from its first
-    token."""
+    that one, until it begins the next). Any other start inside a block, and a start beyond the length (tokens are missing
+    or no longer held as given), shows in _abi.raise_on_status: the sequence stays as it was if the block of `start` would
+    have stayed incomplete; else other tokens stand in their place, and every call that reaches a block without its own
+    reports so, until that is written anew. So does a read or attention over tokens that were never appended."""
     if k.ndim != 4 or k.shape != v.shape:
         raise ValueError('Expected k, v [B,S,H,D]')
     b, s, h, d = k.shape

@@ -227,3 +227,62 @@ def test_where_each_byte_lies(d):
         want[..., place.reshape(-1)] = (blocks + 128).to(torch.uint8).reshape(b, h, 2, 64 * d)
         assert torch.equal(got[:, :, :2].cpu(), want)
         assert torch.equal(scales[:, :, :2].cpu(), torch.ones(b, h, 2))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('held', [0, 1, 64, 100, 128])
+def test_tokens_that_were_never_appended_are_reported_on_block_boundaries_too(dtype, held):
+    from qwen3_triton.inference import quantized as Q
+    h, d, t = 1, 64, 600
+    k, v = tokens(1, t, h, d, dtype, 70)
+    cache = make(1, h, t, d, dtype)
+    if held:
+        Q.append(part(k, 0, held), part(v, 0, held), cache, 0)
+    cache.keys.fill_(7), cache.values.fill_(9), cache.key_scales.fill_(1), cache.value_scales.fill_(1)     # finite, whatever is read
+    if held:
+        Q.append(part(k, 0, held), part(v, 0, held), cache, 0)
+    marks = cache.marks.clone()
+    for end in (64, 192, 256):
+        for call in (lambda: Q.read(cache, end), lambda: Q.read(cache, lengths(end), 0, end), lambda: Q.read(cache, end, end - 1),
+                     lambda: Q.attention(randn((1, 1, 2, d), 1, dtype).cuda(), cache, end - 1),
+                     lambda: Q.attention(randn((1, 40, 2, d), 1, dtype).cuda(), cache, end - 40)):
+            call()
+            assert reported() == (end > held), end
+    Q.append(part(k, 192, 200), part(v, 192, 200), cache, 192)                # a gap before a block: nothing is written
+    assert reported() and torch.equal(cache.marks, marks)
+    Q.append(part(k, 192, 300), part(v, 192, 300), cache, 192)                # blocks beyond the gap: reported until it is filled
+    assert reported()
+    for s in (1, 40):
+        Q.attention(randn((1, s, 2, d), 1, dtype).cuda(), cache, 300 - s)
+        assert reported()
+    Q.read(cache, 300, 256)
+    assert reported()
+    if held >= 64:
+        expect_read(Q.read(cache, 64)[0][0], k[0], 64)                        # what was whole is whole
+        assert not reported()
+    Q.append(part(k, 300, 310), part(v, 300, 310), cache, 300)
+    assert reported()
+    first = held // 64 * 64                                                   # the ring holds blocks 3 and 4
+    Q.append(part(k, first, 310), part(v, first, 310), cache, first)
+    assert not reported()
+    expect_read(Q.read(cache, 310)[0][0], k[0], 310)
+    q = randn((1, 40, 2, d), 2, dtype)
+    expect_attention(Q.attention(q.cuda(), cache, 270)[0], q[0], k[0, :310], v[0, :310], 270, dtype)
+    assert not reported()
+
+
+def test_a_gap_is_filled_from_where_the_sequence_ended():
+    from qwen3_triton.inference import quantized as Q
+    dtype, h, d = torch.bfloat16, 1, 64
+    k, v = tokens(1, 300, h, d, dtype, 71)
+    cache = make(1, h, 300, d, dtype)
+    Q.append(part(k, 0, 100), part(v, 0, 100), cache, 0)
+    Q.append(part(k, 128, 192), part(v, 128, 192), cache, 128)                # block 2; block 1 is held up to token 100
+    assert reported()
+    Q.read(cache, 192)
+    assert reported()
+    Q.append(part(k, 100, 200), part(v, 100, 200), cache, 100)
+    assert not reported()
+    expect_read(Q.read(cache, 200)[0][0], k[0], 200)
+    expect_read(Q.read(cache, 200)[1][0], v[0], 200)
+    assert not reported()
