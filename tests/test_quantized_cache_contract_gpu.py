@@ -286,3 +286,78 @@ def test_a_gap_is_filled_from_where_the_sequence_ended():
     expect_read(Q.read(cache, 200)[0][0], k[0], 200)
     expect_read(Q.read(cache, 200)[1][0], v[0], 200)
     assert not reported()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_every_quotient_of_significands_rounds_as_in_exact_arithmetic(dtype):
+    """A block for every significand A of the largest magnitude, with all x = X 2^-k of the type below it: quotients 127 X 2^-k / A
+    as near to a tie as they come (0.50000192 for X = 2047, k = 8, A = 2031), in whole numbers on the host's side."""
+    from qwen3_triton.inference import quantized as Q
+    bits, d = (8, 128) if dtype == torch.bfloat16 else (11, 128)
+    low = 1 << (bits - 1)
+    a = torch.arange(low, 2 * low, device='cuda')
+    row, dim = torch.arange(64, device='cuda')[:, None], torch.arange(d, device='cuda')[None]
+    places = ((row // 8 * (d // 64) + dim // 64) * 512 + row % 8 * 64 + dim % 64, dim * 64 + row // 2 % 4 * 16 + row // 8 * 2 + row % 2)
+    cache = make(1, low, 64, d, dtype)
+    given, wanted = [], []
+    for first in (0, 1):                                                      # keys: k = 0..7, values: k = 1..8
+        k = torch.arange(first, first + 8, device='cuda')[:, None]
+        x = torch.arange(low, 2 * low, device='cuda')[None].expand(8, low)
+        x, k = x.reshape(1, -1), k.expand(8, low).reshape(1, -1)              # [1, 8 low]
+        over = a[:, None] << k                                                # the quotient is 127 x / over
+        x = torch.where(x <= over, x, torch.zeros_like(x))
+        whole = (254 * x + over) // (2 * over)
+        whole -= (((254 * x + over) % (2 * over) == 0) & (whole % 2 == 1)).long()            # halves to even
+        value = x.double() * torch.exp2(-k.double())
+        sign = 1 - 2 * (torch.arange(x.shape[1], device='cuda') % 3 == 0).long()
+        fill = torch.zeros(low, 64 * d, dtype=torch.float64, device='cuda')
+        want = torch.zeros(low, 64 * d, dtype=torch.int64, device='cuda')
+        n = min(x.shape[1], 64 * d - 1)
+        fill[:, 1:n + 1], want[:, 1:n + 1] = (value * sign)[:, :n], (whole * sign)[:, :n]
+        fill[:, 0], want[:, 0] = a.double(), 127
+        given.append(fill.to(dtype).view(low, 64, d).transpose(0, 1)[None].contiguous())
+        assert torch.equal(given[-1].double(), fill.view(low, 64, d).transpose(0, 1)[None])
+        wanted.append(want)
+    Q.append(*given, cache, 0)
+    for got, want, place in zip((cache.keys, cache.values), wanted, places):
+        assert torch.equal(got[0, :, 0][:, place.reshape(-1)].long() - 128, want)
+
+
+def test_scores_far_from_zero_that_are_exact():
+    """Scores of several thousand that fp32 holds exactly: equal ones average the values, and of two sizes the larger takes all."""
+    from qwen3_triton.inference import quantized as Q
+    for s in (1, 3, 40):
+        for t, later in ((150, 0), (1000, 0), (150, 100), (1000, 700)):
+            dtype, d = torch.bfloat16, 64
+            k, v = torch.zeros(1, t, 1, d), randn((1, t, 1, d), 81)
+            k[..., 0] = 127 * 64.0                                            # n = 127 with a scale of 64, and 8128 as given
+            if later:
+                k[:, later:, :, 0] = -127 * 64.0
+            q = torch.zeros(1, s, 4, d)
+            q[..., 0] = 4.0                                                   # scores of 4064, or -4064
+            k, v, q = k.to(dtype), v.to(dtype), q.to(dtype)
+            cache = make(1, 1, t, d, dtype)
+            Q.append(k.cuda(), v.cuda(), cache, 0)
+            out = Q.attention(q.cuda(), cache, t - s)[0].double().cpu()
+            want, scale, _ = OQ.attention(q[0], OQ.held(k[0], t), OQ.held(v[0], t), t - s)
+            # with scale * log2(e) in fp32 a score is off by 2^-23 of itself at most, 4064 * 1.45 * 2^-23 < 2^-10 in the exponent, the same
+            # for equal scores; the weights' and the result's rounding as for any scores
+            bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -9) * (scale + want.abs())
+            assert float(((out - want).abs() - bound).max()) <= 0, (s, t, later)
+
+
+@pytest.mark.parametrize('capacity', [1001, 5000, 300000])
+def test_a_cache_much_longer_than_its_sequences(capacity):
+    """With lengths on the device a call is cut for the whole capacity: most pieces then have no tokens."""
+    from qwen3_triton.inference import quantized as Q
+    dtype, b, h, hq, d = torch.bfloat16, 3, 2, 8, 128
+    held = (1001, 64, 65)
+    k, v = tokens(b, 1001, h, d, dtype, 91)
+    cache = make(b, h, capacity, d, dtype)
+    Q.append(k.cuda(), v.cuda(), cache, 0, lengths(*held))
+    for s in (1, 4, 30):
+        q = randn((b, s, hq, d), 92, dtype)
+        out = Q.attention(q.cuda(), cache, lengths(*(n - s for n in held)))
+        for i, n in enumerate(held):
+            expect_attention(out[i], q[i], k[i, :n], v[i, :n], n - s, dtype)
+    assert not reported()
