@@ -5,7 +5,9 @@
 // the scale of the values is part of the exponent, so the weights that meet the integers lie in [0, 1] whatever the blocks'
 // scales are, and numerator and denominator keep a running reference each (m, ml). Weights are rounded to fp16 after a
 // factor of 2^15: 11 bits down to 2^-29 of the largest. Integers are exact in fp16; queries in bf16 are taken to fp16 by a
-// power of two per row, and the incomplete block's tokens by one per block. Products accumulate in fp32.
+// power of two per row, and the incomplete block's tokens by one per block: their elements reach 2^15 where integers reach 127,
+// so their weights have 8 bits less of that room, and one 2^-39 of the block's largest (2^-29 where the mark holds a larger one)
+// counts as zero. Products accumulate in fp32.
 // The denominator adds up the weights too, block by block, with vs taken out again. Where vs is below 2^-kFar of the largest so
 // far and the block's largest weight below 2^-kFar, the block counts with a larger vs, such that this weight is 2^-kFar: in fp16
 // its weights are zero with either, and its share of the denominator does not flush. The last factor 2^{m - ml} / sum reaches beyond fp32's exponents and is applied as two halves.
@@ -136,8 +138,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // as tensor-core fragments without bank conflicts. Keys (and value columns) are the 16 rows of the MMA tile and the query rows
 // its 8 columns, so a group of up to 8 query heads fills the tile: S^T = K Q^T, O^T = V^T P^T. Short sequences are a matter of
 // latency: the first copies leave before anything else is looked up, and products that follow one another go to different
-// accumulators. 32 query / 8 kv heads of 128 in bf16: 64 sequences of 8001 tokens 158 us (6.6 TB/s), 4 of 131001 161 us, one of
-// 1501 9 us, of which a CTA needs 1 us until its copies have left and 1.5 us for its first block.
+// accumulators. 32 query / 8 kv heads of 128 in bf16: 64 sequences of 8001 tokens 157 us (6.7 TB/s), 4 of 131001 160 us, one of
+// 1501 9.5 us, of which a CTA needs 1 us until its copies have left and 1.5 us for its first block.
 constexpr int ring_bytes(int warps) { return warps == 4 ? 24576 : 16384; }   // per warp
 
 template <typename T, int D, int NT, int WARPS>
@@ -555,10 +557,11 @@ attention_split_kernel(const AttendParams p) {
 //                the scores they came from, as the A operand of the second product. Only when a row outgrows its reference are
 //                the sums in tensor memory rescaled.
 //   warps 12, 13 issue the products, one tile each: while one tile's weights are computed, the other tile's products run
-// 32 query / 8 kv heads of 128 in bf16: 512 tokens over 32000 292 us (930 TFLOP/s; products alone 163 us at the measured rate), two
-// prompts of 4096 325 us. Bound by the chain scores -> exponentials -> weights -> products of a tile: about 4000 cycles per 256 x
-// 128 against 2050 of products, the exponentials of the two tiles taking turns (297 us; at once 385 us for the first case), and
-// by some 20000 cycles per CTA before its first and after its last step.
+// 32 query / 8 kv heads of 128 in bf16: 512 tokens over 32000 302 us (900 TFLOP/s; products alone 163 us at the measured rate), two
+// prompts of 4096 332 us. Bound by the chain scores -> exponentials -> weights -> products of a tile, which has one place for scores
+// and weights: about 4000 cycles per 256 x 128 against 2050 of products, and as many of shared memory (256 KB per step, operands
+// read and widened tiles written, at 128 bytes a cycle). The exponentials of the two tiles take turns (when that was built, the
+// first case took 297 us, at once 385). Some 20000 cycles per CTA pass before its first and after its last step.
 // Registers move from the other warps to the softmax's: 128 threads x (120 + 56) + 256 x 168 = 512 x 128 at launch.
 constexpr int kPromptThreads = 16 * 32;
 constexpr int kPromptRows = 256;
@@ -1046,8 +1049,10 @@ attention_merge_kernel(const float* __restrict__ part, const float* __restrict__
 }
 
 // How a call is cut. Up to 16 rows: rows in one tile of 8 or 16, the units in `splits` pieces, for CTAs of eight warps (one per
-// SM) where they all run at once, else of four (two per SM). More rows: tiles of 256 rows, key tiles of 128 tokens in `splits`
-// pieces. The number of pieces is the one with the shortest time in a model of it: waves of CTAs times what a CTA takes - a fixed
+// SM) where there are no more (sequence, head) pairs than SMs, else of four (two per SM). More rows: tiles of 256 rows, key tiles
+// of 128 tokens in `splits` pieces, also where the rows are few and the cache is long (8 sequences of 32005 tokens, the last 5 of
+// them new, 32 / 8 heads: 20 rows, 325 us; the cache could be read in 81; 4 new ones, 16 rows: 102 us). `longest` is the capacity
+// where the lengths are on the device: 64 sequences of 1001 tokens take 33 us in a cache of 8192 tokens, 75 us in one of 32768. The number of pieces is the one with the shortest time in a model of it: waves of CTAs times what a CTA takes - a fixed
 // part and its share of the steps - and a second launch where there are pieces to merge - up to 8 pieces of few rows are a
 // cluster of CTAs, which merges them over its shared memory; all in units of one step (a block per warp, or a key tile), as
 // measured: few rows 2.5 + blocks per warp, and 1.5 for the merge, 0.5 within a cluster; many rows 8 + key tiles, and 2.
