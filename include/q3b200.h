@@ -506,7 +506,8 @@ int q3_select_tokens(const void* logits, int64_t B, int64_t V, int64_t* ids, int
  * Lengths: `start` tokens are held before the call, the same for all sequences, or starts[b] if `starts` is not NULL
  * (int64 on the device: a captured call may then be replayed with other lengths). Of the S new tokens of sequence b
  * the first counts[b] are real (all S if `counts` is NULL); the rest is padding, which need not fit the capacity. A `start` from
- * the host is refused where start + S does not fit, or with `counts` start alone. A sequence whose lengths do not fit sets Q3_STATUS_CACHE_RANGE and is left alone (its outputs are zero). */
+ * the host is refused where start + S does not fit, or with `counts` start alone. A sequence whose lengths do not fit sets
+ * Q3_STATUS_CACHE_RANGE and is left alone (its outputs are zero). */
 typedef struct q3_quantized_cache {
   void* keys;
   void* values;

@@ -10,7 +10,8 @@
 // counts as zero. Products accumulate in fp32.
 // The denominator adds up the weights too, block by block, with vs taken out again. Where vs is below 2^-kFar of the largest so
 // far and the block's largest weight below 2^-kFar, the block counts with a larger vs, such that this weight is 2^-kFar: in fp16
-// its weights are zero with either, and its share of the denominator does not flush. The last factor 2^{m - ml} / sum reaches beyond fp32's exponents and is applied as two halves.
+// its weights are zero with either, and its share of the denominator does not flush. The last factor 2^{m - ml} / sum reaches
+// beyond fp32's exponents and is applied as two halves.
 #include "quantized_cache.cuh"
 #include "tcgen05.cuh"
 #include <math_constants.h>
@@ -1052,10 +1053,11 @@ attention_merge_kernel(const float* __restrict__ part, const float* __restrict__
 // SM) where there are no more (sequence, head) pairs than SMs, else of four (two per SM). More rows: tiles of 256 rows, key tiles
 // of 128 tokens in `splits` pieces, also where the rows are few and the cache is long (8 sequences of 32005 tokens, the last 5 of
 // them new, 32 / 8 heads: 20 rows, 325 us; the cache could be read in 81; 4 new ones, 16 rows: 102 us). `longest` is the capacity
-// where the lengths are on the device: 64 sequences of 1001 tokens take 33 us in a cache of 8192 tokens, 75 us in one of 32768. The number of pieces is the one with the shortest time in a model of it: waves of CTAs times what a CTA takes - a fixed
-// part and its share of the steps - and a second launch where there are pieces to merge - up to 8 pieces of few rows are a
-// cluster of CTAs, which merges them over its shared memory; all in units of one step (a block per warp, or a key tile), as
-// measured: few rows 2.5 + blocks per warp, and 1.5 for the merge, 0.5 within a cluster; many rows 8 + key tiles, and 2.
+// where the lengths are on the device: 64 sequences of 1001 tokens take 33 us in a cache of 8192 tokens, 75 us in one of 32768.
+// The number of pieces is the one with the shortest time in a model of it: waves of CTAs times what a CTA takes - a fixed part and
+// its share of the steps - and a second launch where there are pieces to merge - up to 8 pieces of few rows are a cluster of CTAs,
+// which merges them over its shared memory; all in units of one step (a block per warp, or a key tile), as measured: few rows 2.5
+// + blocks per warp, and 1.5 for the merge, 0.5 within a cluster; many rows 8 + key tiles, and 2.
 // Eight warps against two CTAs of four, us: 4 x 131001 tokens 160 / 174, one sequence of 32001 17.6 / 20.3, of 301 7.0 / 8.3; but
 // 64 of 8001 169 / 158 and of 1001 38 / 33: uneven waves cost more when a CTA has the SM.
 struct Plan {

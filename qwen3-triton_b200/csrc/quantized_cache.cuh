@@ -3,8 +3,9 @@
 // Tokens are held in blocks of 64. A complete block of one (sequence, kv head) is 64 * D bytes of keys and as many of
 // values, with one fp32 scale each; the last 128 tokens are also kept as they were given, in a ring of two
 // blocks ("recent"), so that the incomplete block is exact and a block gets its scale from its own tokens,
-// however the appends were cut (marks say what of it can be relied on: tokens of the last two blocks). Both forms store their elements in the order in which the tensor-core fragments of
-// attention read them, so that a warp's loads are consecutive 16-byte pieces:
+// however the appends were cut (marks say what of it can be relied on: tokens of the last two blocks). Both forms store
+// their elements in the order in which the tensor-core fragments of attention read them, so that a warp's loads are
+// consecutive 16-byte pieces:
 //   keys    [token / 8][dim / 64][token % 8][dim % 64]      lane (g, t) of a warp: token 8i + g, dims 64c + 16t .. +15
 //   values  [dim][(token / 2) % 4][token / 8][token % 2]    lane (g, t): dim 8m + g, tokens 8i + 2t, 8i + 2t + 1, i = 0..7
 // (the pair of tokens a lane holds of the value fragment is the pair of scores it holds of the score fragment).
